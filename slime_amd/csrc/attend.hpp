@@ -277,7 +277,8 @@ struct Rows {
     }
 };
 
-// An address that every lane of the wave has alike, in scalar registers.
+// An address that every lane of the wave has alike, in scalar registers that vector instructions
+// may have written just before.
 __device__ __forceinline__ const unsigned char* uniform(const unsigned char* p) {
     const unsigned long long v = reinterpret_cast<unsigned long long>(p);
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
@@ -320,7 +321,7 @@ struct Stage : Fill<Tile<T, DP, kRows>::kRowB, kRows, kThr> {
                     v[i][0] = load16(q + off);
                     v[i][1] = load16(q + off + 16);
                 } else
-                    dma16_lds(q, off, at + 16 * i * kThr);
+                    dma16_lds_v(q, off, at + 16 * i * kThr);
             }
         } else if (!kSplit && s.direct) {
             const unsigned at = lds_addr(tile) + 16 * __builtin_amdgcn_readfirstlane(tid & ~63);
@@ -328,7 +329,7 @@ struct Stage : Fill<Tile<T, DP, kRows>::kRowB, kRows, kThr> {
             for (int i = 0; i < kN; ++i) {
                 const unsigned off =
                     (unsigned)min(row(i, tid), n - 1) * (unsigned)s.row_b + (unsigned)(kGlobalB * chunk(i, tid));
-                if (chunk(i, tid) * kElems < D) dma16_lds(uniform(p), off, at + 16 * i * kThr);
+                if (chunk(i, tid) * kElems < D) dma16_lds_v(uniform(p), off, at + 16 * i * kThr);
             }
         } else {
             uint4 w[kN];

@@ -141,10 +141,27 @@ __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0x0F70);
 // 32-bit and the compiler does not make every later LDS read wait for all such loads
 // in flight (it cannot tell which buffer they fill): each kernel waits for them
 // itself (vmcnt) before the barrier that publishes them. base and lds are uniform.
+//
+// A memory instruction reads a scalar register right five wait states after a vector instruction
+// wrote it (v_readfirstlane, v_readlane, a compare). The compiler adds them between its own
+// instructions but does not look into the asm, which has two: base comes from scalar arithmetic
+// alone here, and dma16_lds_v takes the others (tests/test_wait_states.py reads every kernel's
+// listing).
 __device__ __forceinline__ void dma16_lds(const void* base, unsigned voff, unsigned lds) {
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
         "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2"
+        :
+        : "s"(lds), "v"(voff), "s"(base)
+        : "memory", "m0");
+}
+
+// As dma16_lds, for a base that vector instructions may have written: s_mov and four of s_nop.
+__device__ __forceinline__ void dma16_lds_v(const void* base, unsigned voff, unsigned lds) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 3\n\t"
         "global_load_lds_dwordx4 %1, %2"
         :
         : "s"(lds), "v"(voff), "s"(base)
