@@ -274,12 +274,16 @@ __global__ __launch_bounds__(kThreads) void attend_keys_kernel(const AttendArgs 
         sk.finish(lds_k[buf], tid);
         sv.finish(lds_v[buf], tid);
     };
+    // A split without tiles goes straight to the waves' results, which lie in the tiles' place: it
+    // writes nothing there before, so that no barrier is needed between.
+    if (t0 < t1) {
 #pragma unroll
-    for (int i = 0; i < kBufs; ++i) {
-        Kv::St::clear_pad(lds_k[i], a.D, tid);
-        Kv::St::clear_pad(lds_v[i], a.D, tid);
+        for (int i = 0; i < kBufs; ++i) {
+            Kv::St::clear_pad(lds_k[i], a.D, tid);
+            Kv::St::clear_pad(lds_v[i], a.D, tid);
+        }
+        issue(t0, 0);
     }
-    if (t0 < t1) issue(t0, 0);
 
     Op<T> q[1][kRowSteps<T, DP>];
     Row row;
