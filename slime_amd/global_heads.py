@@ -36,21 +36,25 @@ class GlobalHeads:
         self.freqs = rotation_freqs(ca.D, base, axes=2)
         n = torch.arange(ca.G * ca.G, device="cuda")
         self.positions = torch.stack((n // ca.G, n % ca.G), -1).to(torch.int32).expand(ca.B, -1, -1)
-        self._saved = None
+        self._saved = self._gains = None
 
     def _heads(self, t):
         ca = self.ca
         return t.view(ca.B, ca.G * ca.G, ca.H, ca.D)
 
     def forward(self, x, alive=None):
-        """The heads' output for states x; ``alive``: bool [B, G, G], the cells that are seen."""
+        """The heads' output for states x; ``alive``: bool [B, G, G], the cells that are seen. What
+        ``backward`` needs is kept here, apart from what the caller has: the output, the mask and
+        the gains may be changed in place before it."""
         q0, k0, v = (self._heads(t) for t in self.ca.project(x))
         if alive is not None:
-            alive = alive.reshape(self.ca.B, -1)
-        q, k = qk_norm_rotate(q0, k0, self.wq, self.wk, self.positions, self.freqs, eps=self.eps)
+            alive = alive.reshape(self.ca.B, -1).clone()
+        gains = self.wq.clone(), self.wk.clone()
+        q, k = qk_norm_rotate(q0, k0, *gains, self.positions, self.freqs, eps=self.eps)
         out, lse = attend(q, k, v, alive=alive)
         self._saved = (q0, k0, q, k, v, out, lse, alive)
-        return out.view(self.ca.state_shape)
+        self._gains = gains
+        return out.clone().view(self.ca.state_shape)
 
     def backward(self, grad):
         """Gradients of the projections of the last forward, planes as states -> (dP, dI, dV); of the
@@ -59,7 +63,7 @@ class GlobalHeads:
             raise RuntimeError("backward without a forward")
         q0, k0, q, k, v, out, lse, alive = self._saved
         dq, dk, dv = attend_backward(self._heads(grad), q, k, v, out, lse, alive=alive)
-        dP, dI, self.dwq, self.dwk = qk_norm_rotate_backward(dq, dk, q0, k0, self.wq, self.wk, self.positions,
+        dP, dI, self.dwq, self.dwk = qk_norm_rotate_backward(dq, dk, q0, k0, *self._gains, self.positions,
                                                              self.freqs, eps=self.eps)
         return tuple(t.view(self.ca.state_shape) for t in (dP, dI, dv))
 
