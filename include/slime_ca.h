@@ -391,7 +391,7 @@ typedef struct {
  * the gains w (device fp32 [D]: wq, wk), and its pairs (u, v) turned by the angle
  * t = position * freq: (n_u cos t - n_v sin t, n_u sin t + n_v cos t). Angles are exact
  * to 2^-53 turns per position, also at positions near 2^31. q_out and k_out may be q and
- * k themselves (same strides). */
+ * k themselves (same strides). B N D is below 2^35. */
 int slime_ca_qk_norm_rotate(const slime_ca_norm_config* config, const slime_ca_heads* q,
                             const slime_ca_heads* k, const float* wq, const float* wk,
                             const slime_ca_heads* q_out, const slime_ca_heads* k_out, void* stream);
@@ -433,7 +433,9 @@ typedef struct {
  * bits: errors are as of fp32 products, and a value above 3.39e38 or infinite counts as NaN.
  * A query that sees no key gives 0 and -inf. One
  * query or few over many keys are split over the device, through the workspace (device,
- * 16-byte aligned, slime_ca_attend_workspace bytes for the current device; may be 0). */
+ * 16-byte aligned, slime_ca_attend_workspace bytes for the current device; may be 0). A batch
+ * of more workgroups than one launch takes (2^24, of one head's queries each) goes in several;
+ * one entry that exceeds a launch is SLIME_EINVAL. */
 int slime_ca_attend_workspace(const slime_ca_attend_config* config, int backward, size_t* bytes);
 int slime_ca_attend(const slime_ca_attend_config* config, const slime_ca_heads* q, const slime_ca_heads* k,
                     const slime_ca_heads* v, const slime_ca_heads* out, float* lse, void* workspace,

@@ -1171,6 +1171,9 @@ static int shared_heads(int Hq, int Hkv, int D, int dtype) {
     return SLIME_OK;
 }
 
+// HIP takes fewer than 2^32 threads along an axis of a grid; workgroups here have 256.
+static constexpr long long kMostWorkgroups = (1LL << 24) - 1;
+
 static int workspace_for(size_t need, const void* workspace, size_t bytes) {
     if (need == 0) return SLIME_OK;
     if (!workspace || bytes < need)
@@ -1219,6 +1222,9 @@ int slime_ca_qk_norm_rotate(const slime_ca_norm_config* config, const slime_ca_h
     a.ok = heads_arg(k_out);
     a.wq = wq;
     a.wk = wk;
+    if (norm_blocks(a) > kMostWorkgroups)
+        return fail(SLIME_EINVAL, "B=%d times N=%d rows of heads of %d exceed one launch (%lld workgroups)", a.B, a.N,
+                    a.D, kMostWorkgroups);
     HIP_TRY(launch_norm_rotate(config->dtype, a, (hipStream_t)stream));
     return SLIME_OK;
 }
@@ -1271,7 +1277,8 @@ static int device_cus() {
 }
 
 // The arguments without tensors, and how many workgroups share the keys of a row tile (and,
-// backward, the rows of a key tile) on the current device.
+// backward, the rows of a key tile) on the current device. A batch of more workgroups than a launch
+// takes goes in slices: a->B is the entries of one, and the plan and the workspace are a slice's.
 static int attend_args(const slime_ca_attend_config* c, bool backward, AttendArgs* a, AttendPlan* p) {
     if (!c) return fail(SLIME_EINVAL, "config is NULL");
     if (int rc = shared_heads(c->Hq, c->Hkv, c->D, c->dtype)) return rc;
@@ -1304,15 +1311,25 @@ static int attend_args(const slime_ca_attend_config* c, bool backward, AttendArg
     a->splits = a->row_splits = 1;
     *p = AttendPlan{128, 1, 1};
     if (a->B == 0) return SLIME_OK;
+    auto workgroups = [&] {
+        return backward ? attend_grad_workgroups(c->dtype, *a, *p) : attend_workgroups(*a, *p);
+    };
+    // One entry, not split.
+    a->B = 1;
+    p->rows = !backward && (long long)a->Nq * group <= 32 ? 32 : 128;
+    if (workgroups() > kMostWorkgroups)
+        return fail(SLIME_EINVAL, "Nq=%d, Nk=%d, Hq=%d, Hkv=%d: one batch entry exceeds one launch (%lld workgroups)",
+                    a->Nq, a->Nk, a->Hq, a->Hkv, kMostWorkgroups);
     const int n_cu = device_cus();
     if (n_cu < 1) return fail(SLIME_ENODEV, "no HIP device visible");
-    const long long rows = (long long)a->Nq * group;
-    // The smallest tiles have 32 rows or 128 keys (twice, in two roles); a grid holds below 2^31
-    // workgroups of both.
-    if ((double)a->B * a->Hkv * (rows / 32 + 1.0) > 1.0e9 || (double)a->B * a->Hkv * (a->Nk / 64 + 1.0) > 1.0e9)
-        return fail(SLIME_EINVAL, "B=%d, Hkv=%d, Nq=%d, Nk=%d need more than 2^31 workgroups", a->B, a->Hkv, a->Nq,
-                    a->Nk);
-    *p = backward ? attend_grad_plan(c->dtype, *a, n_cu) : attend_plan(c->dtype, *a, n_cu);
+    for (a->B = c->B;; a->B = a->B / 2 + a->B % 2) {
+        *p = backward ? attend_grad_plan(c->dtype, *a, n_cu) : attend_plan(c->dtype, *a, n_cu);
+        if (workgroups() <= kMostWorkgroups) break;
+        if (a->B == 1) {
+            p->splits = p->row_splits = 1;
+            break;
+        }
+    }
     a->splits = p->splits;
     a->row_splits = p->row_splits;
     return SLIME_OK;
@@ -1327,6 +1344,23 @@ static size_t attend_workspace(const AttendArgs& a, bool backward) {
     if (backward && a.row_splits > 1) n += a.row_splits * keys * 2 * D;
     if (backward) n += rows;
     return n * sizeof(float);
+}
+
+// Launches the slices of a batch of B entries, in order: each the next a.B of them.
+static int launch_slices(hipError_t (*launch)(int, const AttendArgs&, const AttendPlan&, hipStream_t), int dtype,
+                         AttendArgs a, const AttendPlan& p, int B, void* stream) {
+    const long long size = dtype == SLIME_BF16 ? 2 : 4, n = a.B;
+    for (long long b = 0; b < B; b += n) {
+        a.B = (int)(B - b < n ? B - b : n);
+        HIP_TRY(launch(dtype, a, p, (hipStream_t)stream));
+        if (b + n >= B) break;
+        for (HeadsArg* t : {&a.q, &a.k, &a.v, &a.out, &a.gout, &a.gq, &a.gk, &a.gv})
+            if (t->data) t->data = static_cast<char*>(t->data) + n * t->batch * size;
+        if (a.lse) a.lse += n * a.Hq * a.Nq;
+        if (a.lengths) a.lengths += n;
+        if (a.alive) a.alive += n * a.alive_batch;
+    }
+    return SLIME_OK;
 }
 
 int slime_ca_attend_workspace(const slime_ca_attend_config* config, int backward, size_t* bytes) {
@@ -1356,8 +1390,7 @@ int slime_ca_attend(const slime_ca_attend_config* config, const slime_ca_heads* 
     a.out = heads_arg(out);
     a.lse = lse;
     a.part = static_cast<float*>(workspace);
-    HIP_TRY(launch_attend(config->dtype, a, p, (hipStream_t)stream));
-    return SLIME_OK;
+    return launch_slices(launch_attend, config->dtype, a, p, config->B, stream);
 }
 
 int slime_ca_attend_backward(const slime_ca_attend_config* config, const slime_ca_heads* grad_out,
@@ -1390,9 +1423,7 @@ int slime_ca_attend_backward(const slime_ca_attend_config* config, const slime_c
     a.part = static_cast<float*>(workspace);
     a.part_kv = a.part + (a.splits > 1 ? a.splits * rows * a.D : 0);
     a.delta = a.part_kv + (a.row_splits > 1 ? a.row_splits * keys * 2 * a.D : 0);
-    hipStream_t s = (hipStream_t)stream;
-    HIP_TRY(launch_attend_grad(config->dtype, a, p, s));
-    return SLIME_OK;
+    return launch_slices(launch_attend_grad, config->dtype, a, p, config->B, stream);
 }
 
 int slime_snapshot_json(const slime_ca* h, const float* conc, const slime_pool* pool, int generation,

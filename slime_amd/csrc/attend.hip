@@ -507,6 +507,12 @@ AttendPlan attend_plan(int dtype, const AttendArgs& a, int n_cu) {
     return p;
 }
 
+double attend_workgroups(const AttendArgs& a, const AttendPlan& p) {
+    const double rows = (double)a.Nq * a.group, heads = (double)a.B * a.Hkv;
+    const double walks = heads * ceil(rows / p.rows) * p.splits + 8;  // whole eights of them (Deal)
+    return p.splits > 1 ? fmax(walks, ceil(heads * rows * (a.D / 4) / kThreads)) : walks;
+}
+
 hipError_t launch_attend(int dtype, const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
     return dtype == 1 ? run_t<bf16_t, bf16_t>(a, p, s) : run_t<split_t, float>(a, p, s);
 }

@@ -562,6 +562,9 @@ struct Walks {
     }
 };
 
+int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+int roles_of(int dtype, int D) { return padded(D) * (dtype == 1 ? 1 : 3) >= 128 ? 2 : 1; }  // kRoles
+
 }  // namespace
 
 AttendPlan attend_grad_plan(int dtype, const AttendArgs& a, int n_cu) {
@@ -573,7 +576,7 @@ AttendPlan attend_grad_plan(int dtype, const AttendArgs& a, int n_cu) {
     // workgroups a CU, us: in bf16 2 x 2048 x 8 x 128 191 -> 179, 1000, 8 over 2 heads of 128, 72 -> 44,
     // 4096 causal, 8 over 2 heads of 64, 132 -> 94; in fp32 2 x 600 x 8 x 64 84 -> 75. Over 82 calls of
     // 51 to 6144 rows and heads of 32 to 128: 12 % less time, 3 % above the best splits of each call.
-    const int planes = dtype == 1 ? 1 : 3, dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128, roles = dp * planes >= 128 ? 2 : 1;
+    const int planes = dtype == 1 ? 1 : 3, dp = padded(a.D), roles = roles_of(dtype, a.D);
     const bool cut = a.window > 0, one_launch = planes == 1 || dp == 32;
     const double slots_q = (one_launch ? 2.0 : 1.0) * n_cu, slots_kv = (one_launch || dp == 64 ? 2.0 : 1.0) * n_cu;
     const long long seen = a.window * (a.causal ? 1LL : 2LL);
@@ -603,6 +606,14 @@ AttendPlan attend_grad_plan(int dtype, const AttendArgs& a, int n_cu) {
                 p.row_splits = kSplits[j];
             }
     return p;
+}
+
+double attend_grad_workgroups(int dtype, const AttendArgs& a, const AttendPlan& p) {
+    const double heads = (double)a.B * a.Hkv, rows = (double)a.Nq * a.group;
+    const double delta = ceil(heads * rows * (a.D * (dtype == 1 ? 2 : 4) / 16) / kThreads);
+    const double walks = heads * (ceil(rows / p.rows) * p.splits + ceil(a.Nk / 128.0) * p.row_splits * roles_of(dtype, a.D)) + 16;
+    const double sums = heads * ((p.splits > 1 ? rows : 0.0) + (p.row_splits > 1 ? 2.0 * a.Nk : 0.0)) * (a.D / 4) / kThreads + 3;
+    return fmax(delta, fmax(walks, sums));
 }
 
 template <typename G>

@@ -294,7 +294,7 @@ Grid backward_grid(const NormArgs& a) {
 
 template <typename T, int kL, bool kAdjacent>
 hipError_t forward(const NormArgs& a, hipStream_t s) {
-    const long long rows = (long long)a.B * a.N, per = kThreads / kL, x = (rows + per - 1) / per;
+    const long long x = norm_blocks(a);
     const int heads = heads_per_thread(a, x);
     hipLaunchKernelGGL((norm_rotate_kernel<T, kL, kAdjacent>), dim3((unsigned)x, (a.Hq + a.Hkv + heads - 1) / heads),
                        dim3(kThreads), 0, s, a, heads);
@@ -328,6 +328,10 @@ hipError_t run_t(const NormArgs& a, bool back, hipStream_t s) {
 
 }  // namespace
 
+long long norm_blocks(const NormArgs& a) {
+    const long long rows = (long long)a.B * a.N, per = kThreads / (a.D / 8);
+    return (rows + per - 1) / per;
+}
 int norm_backward_blocks(const NormArgs& a) {
     const Grid g = backward_grid(a);
     return (int)(g.x * g.y);

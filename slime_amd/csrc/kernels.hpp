@@ -293,6 +293,7 @@ struct NormArgs {
     float* gwq;            // [D]
     float* gwk;
 };
+long long norm_blocks(const NormArgs& a);  // of the forward, along the rows
 int norm_backward_blocks(const NormArgs& a);
 hipError_t launch_norm_rotate(int dtype, const NormArgs& a, hipStream_t s);
 hipError_t launch_norm_rotate_backward(int dtype, const NormArgs& a, hipStream_t s);
@@ -322,8 +323,10 @@ struct AttendPlan {
     int row_splits;        // backward
 };
 AttendPlan attend_plan(int dtype, const AttendArgs& a, int n_cu);
+double attend_workgroups(const AttendArgs& a, const AttendPlan& p);  // of the call's largest launch
 hipError_t launch_attend(int dtype, const AttendArgs& a, const AttendPlan& p, hipStream_t s);
 AttendPlan attend_grad_plan(int dtype, const AttendArgs& a, int n_cu);
+double attend_grad_workgroups(int dtype, const AttendArgs& a, const AttendPlan& p);
 hipError_t launch_attend_grad(int dtype, const AttendArgs& a, const AttendPlan& p, hipStream_t s);
 
 }  // namespace slime

@@ -54,3 +54,61 @@ def test_splits_without_a_tile(D, dtype):
         first = first or (out, lse)
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
     assert not out[3].any() and bool((lse[3] == -math.inf).all())
+
+
+def _living(B, seed):
+    """(lengths, alive) of one key an entry: 0 or 1, and a cell that lives or not."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.rand(2, B, 1, generator=g, device="cuda") < 0.8).unbind(0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_heads_than_a_launch(dtype):
+    """2^21 entries of 8 heads, one query and one key each, in views of one packed product: twice what
+    a launch of 256 threads a head may hold. With one key the output is its value: its weight and their
+    sum are the same number, so in bf16 bit by bit, in fp32 to the product, the quotient and the
+    joining of four waves. The value's gradient is the output's; the score's is 0, but for its two
+    terms of D products each, rounded apart."""
+    import slime_amd
+    B, H, D, dt = 2 ** 21 + 5, 8, 8, DTYPES[dtype]
+    x = _draw((B, 1, 3 * H, D), dt, 1)
+    q, k, v = x[:, :, :H], x[:, :, H:2 * H], x[:, :, 2 * H:]
+    below, lives = _living(B, 2)
+    how = dict(lengths=below[:, 0].int().contiguous(), alive=lives)
+    seen = (below & lives)[:, :, None, None]
+    out, lse = slime_amd.attend(q, k, v, **how)
+    if dt == torch.bfloat16:
+        assert torch.equal(out, v * seen)
+    else:
+        assert bool(((out - v * seen).abs() <= 8 * ref.U32 * v.abs() * seen).all())
+    score = (q.float() * k.float()).sum(-1).transpose(1, 2) / math.sqrt(D)
+    size = (q.float() * k.float()).abs().sum(-1).transpose(1, 2) / math.sqrt(D)
+    live = seen[..., 0].expand_as(lse)
+    assert bool((lse[~live] == -math.inf).all())
+    # the reference's bound for one key, and as many roundings of the sum here
+    bound = ((2 * D + 16) * size + 48 + 8 * score.abs()) * ref.U32
+    assert bool(((lse - score).abs() <= bound)[live].all())
+    gout = _draw(q.shape, dt, 3)
+    dq, dk, dv = slime_amd.attend_backward(gout, q, k, v, out, lse, **how)
+    # 2^(s - lse) is 1 but for their roundings, and bf16's one
+    off = (2 * D + 24) * ref.U32 * (1 + size + lse.abs().nan_to_num(0, 0, 0)).transpose(1, 2)[..., None]
+    u = ref.u_of(dt) * (2 if dt == torch.bfloat16 else 1)
+    assert bool(((dv.float() - gout.float() * seen).abs() <= (off + u) * gout.float().abs()).all())
+    ds = 4 * (D + 4) * ref.U32 * (gout.float() * v.float()).abs().sum(-1, keepdim=True) * 1.01 / math.sqrt(D)
+    for got, other in ((dq, k), (dk, q)):
+        assert bool((got.float().abs() <= ds * other.float().abs() * seen).all())
+
+
+def test_slices_of_a_batch_take_their_own_lengths():
+    """As many heads, none to three keys an entry: entries about the slices' ends are as in a call of
+    them alone."""
+    import slime_amd
+    B, H, D = 2 ** 21 + 5, 8, 8
+    q, k, v = (_draw((B, 1 if i == 0 else 3, H, D), torch.bfloat16, i) for i in range(3))
+    lengths = (torch.arange(B, device="cuda") % 4).int()
+    out, lse = slime_amd.attend(q, k, v, lengths=lengths)
+    n = 1000
+    for at in (0, B // 2 - n // 2, B - n):
+        part = slice(at, at + n)
+        o, s = slime_amd.attend(q[part], k[part], v[part], lengths=lengths[part])
+        assert torch.equal(o, out[part]) and torch.equal(s, lse[part])
