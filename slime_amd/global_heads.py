@@ -87,7 +87,7 @@ class CellHistory:
         self.length = 0
 
     def step(self, x):
-        """Adds state x and returns its heads' output, [B, G, G, C]."""
+        """Adds state x and returns its heads' output, [B, G, G, C]. A step that raises adds nothing."""
         torch = _torch()
         if self.length == self.capacity:
             raise RuntimeError(f"the history holds its {self.capacity} states")
@@ -97,8 +97,8 @@ class CellHistory:
         q, _ = qk_norm_rotate(q, k, self.wq, self.wk, at, self.freqs, eps=self.eps,
                               out=(torch.empty_like(q), self.keys[:, t:t + 1]))
         self.values[:, t:t + 1].copy_(v)
-        self.length = t + 1
         out, _ = attend(q, self.keys[:, :t + 1], self.values[:, :t + 1], causal=True, window=self.window)
+        self.length = t + 1
         return out.view(self.ca.state_shape)
 
 

@@ -45,3 +45,25 @@ def test_changes_between_forward_and_backward(dtype, what):
         got = (*heads.backward(grad), heads.dwq, heads.dwk)
         for a, b, name in zip(got, want, ("dP", "dI", "dV", "dwq", "dwk")):
             assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("fails", ["qk_norm_rotate", "attend"])
+def test_a_history_step_that_raises_adds_no_state(monkeypatch, fails):
+    """The next step is as if the one that raised had not been made."""
+    from slime_amd import CellHistory, global_heads
+    cfg = slime_amd.CAConfig("heads", B=1, G=16, H=8, D=16, dtype="bf16", steps=1, w_std=0.1)
+    with Pseudopod(cfg.B, cfg.G, cfg.H, cfg.D, cfg.dtype, cfg.dt) as ca:
+        ca.set_params(slime_amd.make_params(cfg, seed=1))
+        x = torch.from_numpy(slime_amd.make_state(cfg, seed=2)).cuda().to(ca.torch_dtype)
+        states = [x, ca.forward(x)]
+        plain, past = CellHistory(ca, capacity=2), CellHistory(ca, capacity=2)
+        want = [plain.step(s) for s in states]
+        for s, y in zip(states, want):
+            with monkeypatch.context() as m:
+                def refuse(*_, **__):
+                    raise slime_amd.SlimeError(-1, "no")
+                m.setattr(global_heads, fails, refuse)
+                with pytest.raises(slime_amd.SlimeError):
+                    past.step(x + 1)
+            assert torch.equal(past.step(s), y)
+        assert past.length == 2
