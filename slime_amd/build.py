@@ -1,6 +1,7 @@
 """Builds ``slime_amd/libslime_ca.so`` (the HIP kernels + C ABI) for gfx950, and
 ``slime_amd/libslime_probe.so`` (the ceiling measurements of ``calibrate.py``), and
-``slime_amd/_binding.so`` (the attention calls over torch tensors, host code).
+``slime_amd/_binding.so`` (the attention calls over torch tensors, host code; left out where no
+torch for ROCm is installed, since the library does not need it).
 
 Each source is compiled with hipcc in parallel into ``slime_amd/_build/`` and
 linked into one shared library next to this file. Packed-fp32 instructions are
@@ -52,9 +53,15 @@ def _compile(src: str) -> str:
     return obj
 
 
-def _build_binding() -> None:
+def _torch_folder():
+    """Where a torch for ROCm is installed, or None: a C or C++ host needs the library alone."""
+    spec = importlib.util.find_spec("torch")
+    folder = list(spec.submodule_search_locations)[0] if spec and spec.submodule_search_locations else None
+    return folder if folder and os.path.exists(os.path.join(folder, "lib", "libc10_hip.so")) else None
+
+
+def _build_binding(torch: str) -> None:
     """The CPython module (host code only), against torch's headers and the library just linked."""
-    torch = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
     tmp = BINDING + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-I{os.path.join(os.path.dirname(HERE), 'include')}", f"-I{torch}/include",
@@ -78,15 +85,18 @@ def build(verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
-    _build_binding()
     tmp = PROBE_LIB + ".tmp"
     cmd = [hipcc(), *flags(), "-x", "hip", "-shared", os.path.join(CSRC, "probe.hip"), "-o", tmp]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for probe.hip:\n{r.stderr}")
     os.replace(tmp, PROBE_LIB)
+    torch = _torch_folder()
+    if torch:
+        _build_binding(torch)
     if verbose:
-        print(f"built {LIB}, {BINDING} and {PROBE_LIB}")
+        print(f"built {LIB} and {PROBE_LIB}" + (f" and {BINDING}" if torch else "; no torch for ROCm here, so no "
+                                                f"{BINDING}: slime_amd.attend and its like will raise"))
     return LIB
 
 
