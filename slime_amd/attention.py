@@ -38,16 +38,21 @@ _native = None  # the module of csrc/binding.cpp
 
 
 def load():
-    """The module that makes the calls; raises if it has not been built."""
+    """The module that makes the calls; raises if it has not been built, or for another torch, whose
+    tensors it would misread."""
     global _native
     if _native is None:
         _lib.load()
-        _torch()  # its libraries are what the module links to
+        torch = _torch()  # its libraries are what the module links to
         if not os.path.exists(BINDING_PATH):
             raise ImportError(f"{BINDING_PATH} is missing: build it with `python -m slime_amd.build`")
         spec = importlib.util.spec_from_file_location("slime_amd._binding", BINDING_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
+        built = getattr(module, "torch_version", "unknown")
+        if built != str(torch.__version__):
+            raise ImportError(f"{BINDING_PATH} was built for torch {built}, this is {torch.__version__}: "
+                              "build it again with `python -m slime_amd.build`")
         _native = module
     return _native
 

@@ -15,6 +15,7 @@ from __future__ import annotations
 import concurrent.futures as cf
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -61,10 +62,13 @@ def _torch_folder():
 
 
 def _build_binding(torch: str) -> None:
-    """The CPython module (host code only), against torch's headers and the library just linked."""
+    """The CPython module (host code only), against torch's headers and the library just linked. It
+    holds torch's version, which attention.load compares with the running one's."""
+    with open(os.path.join(torch, "version.py")) as f:
+        version = re.search(r"^__version__\s*=\s*['\"](.+?)['\"]", f.read(), re.M).group(1)
     tmp = BINDING + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-I{os.path.join(os.path.dirname(HERE), 'include')}", f"-I{torch}/include",
+           f'-DSLIME_TORCH="{version}"', f"-I{os.path.join(os.path.dirname(HERE), 'include')}", f"-I{torch}/include",
            f"-I{torch}/include/torch/csrc/api/include", f"-I{sysconfig.get_path('include')}",
            f"-isystem{os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc()))), 'include')}",
            os.path.join(CSRC, "binding.cpp"), f"-L{HERE}", "-l:libslime_ca.so", "-Wl,-rpath,$ORIGIN",
