@@ -367,9 +367,9 @@ int slime_snapshot_json(const slime_ca* ca, const float* chemical_concentration,
  * A tensor is [B][N][heads][D] (N cells or states), of SLIME_F32 or SLIME_BF16, with any
  * strides (in elements) but 1 along D, from any element of an allocation: a plane
  * [B][G][G][C] has row C and head D. Inputs may repeat memory (stride 0) and share it;
- * outputs must not overlap anything, except that slime_ca_qk_norm_rotate may work in
- * place. D is 8, 16, 32, 64 or 128; Hq is a multiple of Hkv, and query head h uses key
- * head h / (Hq / Hkv). */
+ * outputs must not overlap anything, except that q_out, k_out and attention's out may be
+ * q, k and q themselves, at the same strides. D is 8, 16, 32, 64 or 128; Hq is a multiple
+ * of Hkv, and query head h uses key head h / (Hq / Hkv). */
 typedef struct {
     void* data;
     long long batch, row, head;
@@ -390,8 +390,7 @@ typedef struct {
 /* Queries and keys in one pass: each head x normed, n = x w / sqrt(mean(x^2) + eps) with
  * the gains w (device fp32 [D]: wq, wk), and its pairs (u, v) turned by the angle
  * t = position * freq: (n_u cos t - n_v sin t, n_u sin t + n_v cos t). Angles are exact
- * to 2^-53 turns per position, also at positions near 2^31. q_out and k_out may be q and
- * k themselves (same strides). B N D is below 2^35. */
+ * to 2^-53 turns per position, also at positions near 2^31. B N D is below 2^35. */
 int slime_ca_qk_norm_rotate(const slime_ca_norm_config* config, const slime_ca_heads* q,
                             const slime_ca_heads* k, const float* wq, const float* wk,
                             const slime_ca_heads* q_out, const slime_ca_heads* k_out, void* stream);

@@ -111,10 +111,14 @@ def _check_heads(Hq, Hkv, D) -> None:
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads")
 
 
-def _check_output(t, name, like) -> None:
+def _check_output(t, name, like, itself, apart) -> None:
+    """``apart``: what the output may not share memory with, by name; it may be all of ``itself``."""
     _check(t, name, like, like.shape)
     if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name} repeats memory (strides {t.stride()})")
+    for other, x in apart.items():
+        if x is not None and load().overlaps(t, x, other == itself):
+            raise ValueError(f"{name} lies in the memory of {other}")
 
 
 # ---- norm and rotation ---------------------------------------------------------------------
@@ -150,8 +154,9 @@ def _check_norm(q, k, wq, wk, positions, freqs, eps, pairs, out=None, grads=()):
     if pairs not in PAIRS:
         raise ValueError(f"pairs must be one of {sorted(PAIRS)}, got {pairs!r}")
     if out is not None:
-        for t, name, like in zip(out, ("out[0]", "out[1]"), (q, k)):
-            _check_output(t, name, like)
+        inputs = dict(q=q, k=k, wq=wq, wk=wk, positions=positions, freqs=freqs)
+        _check_output(out[0], "out[0]", q, "q", inputs)
+        _check_output(out[1], "out[1]", k, "k", {**inputs, "out[0]": out[0]})
     for g, name, like in zip(grads, ("grad_q", "grad_k"), (q, k)):
         _check(g, name, q, like.shape)
 
@@ -164,7 +169,8 @@ def qk_norm_rotate(q, k, wq, wk, positions, freqs, *, eps: float = 1e-6, pairs: 
     ``positions``: int32 [B, N, 1] (an index), or [B, N, 2] (a cell's y and x: the first half of the
     pairs turns by y, the second by x); any batch and row strides. ``freqs``: float64 [D / 2], radians
     per position of each pair (``rotation_freqs``). ``pairs``: "halves" turns channels (i, i + D / 2),
-    "adjacent" (2i, 2i + 1). ``out``: (q, k) to write, q and k themselves included."""
+    "adjacent" (2i, 2i + 1). ``out``: (q, k) to write; each may be its own input, place by place, and
+    shares no other memory with the arguments."""
     oq, ok = (None, None) if out is None else out
     return _call("norm", stream, (q, k, wq, wk, positions, freqs, eps, pairs, oq, ok),
                  lambda: _check_norm(q, k, wq, wk, positions, freqs, eps, pairs, out))
@@ -202,7 +208,7 @@ def _check_attend(q, k, v, scale, window, align, lengths, alive, out=None, back=
                               or alive.device != q.device or (Nk > 1 and alive.stride(1) != 1)):
         raise ValueError(f"alive must be a bool or uint8 tensor [{B}, {Nk}] with dense rows on {q.device}")
     if out is not None:
-        _check_output(out, "out", q)
+        _check_output(out, "out", q, "q", dict(q=q, k=k, v=v, lengths=lengths, alive=alive))
     if back:
         grad_out, out, lse = back
         _check(grad_out, "grad_out", q, q.shape)
@@ -222,6 +228,9 @@ def attend(q, k, v, *, scale: float | None = None, causal: bool = False, window:
     (``align`` "end": the queries are the last of the keys, as when a history grows) or p = i
     ("start": a padded batch in training); with ``causal`` it sees j <= p, with a ``window`` W > 0
     p - j < W and, unless causal, j - p < W. A query that sees no key gives 0 and -inf.
+
+    ``out``: where to write the output, of q's shape; it may be q itself, and shares no other memory
+    with the arguments.
 
     Few queries over many keys (one new state over a long history) are split over the device."""
     return _call("attend", stream, (q, k, v, scale, causal, window, align, lengths, alive, out),

@@ -19,6 +19,7 @@
 #include <climits>
 #include <cmath>
 
+#include "overlap.hpp"
 #include "slime_ca.h"
 
 namespace {
@@ -82,8 +83,8 @@ struct Args {
         return t;
     }
     // n contiguous values.
-    void* vector(at::ScalarType type, int64_t n) {
-        const Tensor* t = tensor();
+    void* vector(at::ScalarType type, int64_t n, const Tensor** found) {
+        const Tensor* t = *found = tensor();
         ok = ok && t && t->dim() == 1 && t->size(0) == n && t->scalar_type() == type && t->device() == device &&
              t->is_contiguous();
         return ok ? t->data_ptr() : nullptr;
@@ -121,6 +122,26 @@ bool fits(const Tensor& t) {
     return true;
 }
 
+slime::Region region_of(const Tensor& t) {
+    const long long e = (long long)t.element_size();
+    slime::Region r{(long long)(intptr_t)t.data_ptr(), e, (int)t.dim(), {}, {}};
+    for (int d = 0; d < r.dims; ++d) {
+        r.size[d] = t.size(d);
+        r.stride[d] = t.stride(d) * e;
+    }
+    return r;
+}
+// An output apart from an input, or (may_be) the input itself, place by place: each element is read
+// by the workgroup that writes it, and before.
+bool apart(const Tensor& out, const Tensor& in, bool may_be) {
+    if (may_be && out.data_ptr() == in.data_ptr() && out.sizes() == in.sizes()) {
+        bool same = true;
+        for (int d = 0; d < out.dim(); ++d) same = same && (out.size(d) < 2 || out.stride(d) == in.stride(d));
+        if (same) return true;
+    }
+    return !slime::Overlap::of(region_of(out), region_of(in));
+}
+
 Tensor empty_as(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 slime_ca_heads heads_of(const Tensor& t) {
     return slime_ca_heads{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
@@ -148,7 +169,7 @@ PyObject* results(const T&... t) {
 struct Attend {
     slime_ca_attend_config c{};
     slime_ca_heads hq, hk, hv;
-    const Tensor *q, *k, *v;
+    const Tensor *q, *k, *v, *lengths = nullptr, *alive = nullptr;
     explicit Attend(Args& a) {
         q = a.heads(&hq);
         k = a.heads(&hk);
@@ -179,7 +200,7 @@ struct Attend {
         if (!none) {
             a.ok = n->dim() == 1 && n->size(0) == c.B && n->scalar_type() == at::kInt && n->device() == a.device &&
                    n->is_contiguous();
-            if (a.ok) c.lengths = static_cast<const int*>(n->data_ptr());
+            if (a.ok) c.lengths = static_cast<const int*>((lengths = n)->data_ptr());
         }
         const Tensor* m = a.tensor_or_none(&none);
         if (!none && a.ok) {
@@ -187,10 +208,14 @@ struct Attend {
                    (m->scalar_type() == at::kBool || m->scalar_type() == at::kByte) && m->device() == a.device &&
                    (c.Nk < 2 || m->stride(1) == 1);
             if (a.ok) {
-                c.alive = static_cast<const unsigned char*>(m->data_ptr());
+                c.alive = static_cast<const unsigned char*>((alive = m)->data_ptr());
                 c.alive_batch = m->stride(0);
             }
         }
+    }
+    bool takes(const Tensor& out) const {
+        return alike(&out, q) && apart(out, *q, true) && apart(out, *k, false) && apart(out, *v, false) &&
+               (!lengths || apart(out, *lengths, false)) && (!alive || apart(out, *alive, false));
     }
 };
 
@@ -202,7 +227,7 @@ PyObject* attend(PyObject*, PyObject* const* at, Py_ssize_t n) {
     slime_ca_heads ho;
     none = a.left > 0 && *a.at == Py_None;
     const Tensor* given = none ? (a.next(), nullptr) : a.output(&ho);
-    if (!a.ok || (given && !alike(given, x.q))) Py_RETURN_NONE;
+    if (!a.ok || (given && !x.takes(*given))) Py_RETURN_NONE;
     const c10::hip::HIPGuard guard(a.device.index());
     size_t bytes = 0;
     if (int rc = slime_ca_attend_workspace(&x.c, 0, &bytes)) return PyLong_FromLong(rc);
@@ -244,7 +269,7 @@ PyObject* attend_backward(PyObject*, PyObject* const* at, Py_ssize_t n) {
 struct Norm {
     slime_ca_norm_config c{};
     slime_ca_heads hq, hk;
-    const Tensor *q, *k;
+    const Tensor *q, *k, *small[4];  // the gains, positions and frequencies
     const float *wq = nullptr, *wk = nullptr;
     explicit Norm(Args& a) {
         q = a.heads(&hq);
@@ -258,9 +283,9 @@ struct Norm {
         c.Hkv = (int)k->size(2);
         c.D = (int)q->size(3);
         c.dtype = a.dtype;
-        wq = static_cast<const float*>(a.vector(at::kFloat, c.D));
-        wk = static_cast<const float*>(a.vector(at::kFloat, c.D));
-        const Tensor* p = a.tensor();
+        wq = static_cast<const float*>(a.vector(at::kFloat, c.D, &small[0]));
+        wk = static_cast<const float*>(a.vector(at::kFloat, c.D, &small[1]));
+        const Tensor* p = small[2] = a.tensor();
         a.ok = a.ok && p && p->dim() == 3 && p->size(0) == c.B && p->size(1) == c.N &&
                (p->size(2) == 1 || (p->size(2) == 2 && p->stride(2) == 1)) && p->scalar_type() == at::kInt &&
                p->device() == a.device;
@@ -269,9 +294,15 @@ struct Norm {
         c.positions = static_cast<const int*>(p->data_ptr());
         c.pos_batch = p->stride(0);
         c.pos_row = p->stride(1);
-        c.freqs = static_cast<const double*>(a.vector(at::kDouble, c.D / 2));
+        c.freqs = static_cast<const double*>(a.vector(at::kDouble, c.D / 2, &small[3]));
         c.eps = (float)a.number();
         c.adjacent = a.either("halves", "adjacent");
+    }
+    bool takes(const Tensor& oq, const Tensor& ok) const {
+        bool fine = apart(oq, *q, true) && apart(oq, *k, false) && apart(ok, *k, true) && apart(ok, *q, false) &&
+                    apart(oq, ok, false);
+        for (const Tensor* t : small) fine = fine && apart(oq, *t, false) && apart(ok, *t, false);
+        return fine;
     }
 };
 
@@ -285,7 +316,7 @@ PyObject* norm(PyObject*, PyObject* const* at, Py_ssize_t n) {
     if (!none) {
         gq = a.output(&hoq);
         gk = a.output(&hok);
-        a.ok = a.ok && alike(gq, x.q) && alike(gk, x.k);
+        a.ok = a.ok && alike(gq, x.q) && alike(gk, x.k) && x.takes(*gq, *gk);
     }
     if (!a.ok) Py_RETURN_NONE;
     const c10::hip::HIPGuard guard(a.device.index());
@@ -319,9 +350,20 @@ PyObject* norm_backward(PyObject*, PyObject* const* at, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// (output, input, whether it may be the input itself) -> whether they share memory otherwise.
+PyObject* overlaps(PyObject*, PyObject* const* at, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a{at, n};
+    const Tensor *out = a.tensor(), *in = a.tensor();
+    const bool may_be = a.truth();
+    if (!a.ok || out->dim() > slime::Region::kDims || in->dim() > slime::Region::kDims) Py_RETURN_NONE;
+    return PyBool_FromLong(!apart(*out, *in, may_be));
+    END_HANDLE_TH_ERRORS
+}
+
 #define SLIME_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SLIME_FN(attend), SLIME_FN(attend_backward), SLIME_FN(norm), SLIME_FN(norm_backward),
-                         {nullptr, nullptr, 0, nullptr}};
+                         SLIME_FN(overlaps), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Attention calls over torch tensors.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
