@@ -429,7 +429,8 @@ typedef struct {
  * [B][Hq][Nq]), the log of the sum of exp(scale q . k): fp32 sums; bf16 probabilities are
  * rounded to bf16 before they meet v. In fp32 more than 32 rows of a key head (Nq Hq / Hkv)
  * run on the bf16 matrix cores, each value as the sum of three bf16 parts that hold its 24
- * bits: errors are as of fp32 products, and a value above 3.39e38 or infinite counts as NaN.
+ * bits: errors are as of fp32 products but for values below 2^-110, whose parts end at 2^-133
+ * (bf16's smallest), and a value above 3.39e38 or infinite counts as NaN.
  * A query that sees no key gives 0 and -inf. One
  * query or few over many keys are split over the device, through the workspace (device,
  * 16-byte aligned, slime_ca_attend_workspace bytes for the current device; may be 0). A batch

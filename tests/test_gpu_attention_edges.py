@@ -112,3 +112,38 @@ def test_slices_of_a_batch_take_their_own_lengths():
         part = slice(at, at + n)
         o, s = slime_amd.attend(q[part], k[part], v[part], lengths=lengths[part])
         assert torch.equal(o, out[part]) and torch.equal(s, lse[part])
+
+
+@pytest.mark.parametrize("power", [-20, -100, -112, -120, -126])
+def test_small_fp32_values_in_three_parts(power):
+    """Many rows in fp32: each value as three bf16 parts, of which the last ends at bf16's smallest
+    step, 2^-133. So a value is off by half of that at most, beside the reference's bound, and each of a
+    sum's products by half of fp32's smallest, 2^-149."""
+    import slime_amd
+    B, N, H, D = 1, 70, 2, 32
+    q, k, v = (_draw((B, N, H, D), torch.float32, s) for s in (1, 2, 3))
+    v = (v.double() * 2.0 ** power).float()
+    r = ref.Reference(q, k, v, 1 / math.sqrt(D), ref.seen_mask(B, N, N))
+    out, _ = slime_amd.attend(q, k, v)
+    tol = (2 * r.ds + (N + 32) * ref.U32) * (r.p @ r.v.abs()) + ref.U32 * r.out.abs() + 2.0 ** -134 + 6 * N * 2.0 ** -150
+    ref.within(out, r.out.permute(0, 2, 1, 3), tol.permute(0, 2, 1, 3), "out")
+
+
+@pytest.mark.parametrize("value, fits", [(3.38e38, True), (-3.38e38, True), (3.4e38, False), (math.inf, False)])
+def test_the_largest_fp32_values(value, fits):
+    """Above the largest bf16, 3.39e38, a value of many rows in fp32 is NaN, in its channel alone; few
+    rows take every value."""
+    import slime_amd
+    q, k, v = (torch.zeros(1, n, 1, 32, device="cuda") for n in (64, 64, 64))
+    v[0, 3, 0, 5] = value
+    for rows in (64, 8):
+        out, _ = slime_amd.attend(q[:, :rows], k, v)
+        want = torch.full((rows,), value / 64, device="cuda")
+        got = out[0, :, 0, 5]
+        if fits or rows == 8:
+            # 64 equal weights: their product, the sum's quotient and the split's rest
+            assert torch.equal(got, want) or float(((got - want) / want).abs().max()) <= 16 * ref.U32
+        else:
+            assert bool(torch.isnan(got).all())
+        out[0, :, 0, 5] = 0
+        assert not out.any()
