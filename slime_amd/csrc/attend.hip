@@ -237,6 +237,11 @@ __global__ __launch_bounds__(kThreads, DP <= (Elem<T>::kPlanes == 3 ? 64 : 128) 
 }
 
 // ---- few rows: four waves share 32 rows and take 32 keys each of a tile of 128 -------------
+// They wait for memory, so bf16 weights keep 16 bits here: the output's error is its own rounding,
+// 1.4 times that in attend_rows_kernel, whose time more products would add to.
+template <typename T>
+using KeysProbs = typename std::conditional<sizeof(T) == 2, ProbsInTwo, Probs<T>>::type;
+
 template <typename T, int DP, bool kAlive>
 __global__ __launch_bounds__(kThreads) void attend_keys_kernel(const AttendArgs a, const int row_tiles,
                                                                const Deal deal) {
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(kThreads) void attend_keys_kernel(const AttendArgs 
                     for (int i = 0; i < 16; ++i) o[0][d][i] *= fix;
             }
             row.weights(s[0], c);
-            const Probs<T> p[1] = {Probs<T>(s[0])};
+            const KeysProbs<T> p[1] = {KeysProbs<T>(s[0])};
             mma_cols<T, DP, kKeys>(o, vt, 32 * wave, p, lane);
         }
         if (kBufs == 1) {

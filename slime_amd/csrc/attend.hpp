@@ -13,6 +13,8 @@
 // whole group, and the group's gradients of keys and values are summed by the products.
 #pragma once
 
+#include <type_traits>
+
 #include "attend_walk.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -218,13 +220,39 @@ struct Probs<float> {
     __device__ __forceinline__ Probs() {}
     __device__ __forceinline__ explicit Probs(const f32x16& p) : v(p) {}
 };
+// bf16 pairs with what their rounding left, rounded too: at most 2^-16 of each probability, for a
+// second product and five instructions a pair.
+struct ProbsInTwo {
+    Probs<bf16_t> hi, lo;
+    __device__ __forceinline__ explicit ProbsInTwo(const f32x16& p) : hi(p) {
+        f32x16 rest;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint4& h = hi.v[t].p[0];
+            const unsigned w[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                rest[8 * t + 2 * e] = p[8 * t + 2 * e] - bf16lo(w[e]);
+                rest[8 * t + 2 * e + 1] = p[8 * t + 2 * e + 1] - bf16hi(w[e]);
+            }
+        }
+        lo = Probs<bf16_t>(rest);
+    }
+};
+template <typename T>
+__device__ __forceinline__ f32x16 mma_probs(const Op<T>& a, const Probs<T>& p, int s, f32x16 c) {
+    return mma(a, p.v[s], c);
+}
+__device__ __forceinline__ f32x16 mma_probs(const Op<bf16_t>& a, const ProbsInTwo& p, int s, f32x16 c) {
+    return mma(a, p.hi.v[s], mma(a, p.lo.v[s], c));
+}
 
 // acc[n][d][.] += sum over tile rows r0 .. r0 + 31 of tile[row][d] p[n][row][.], in blocks of 32
 // channels d. The tile is read along its columns: transposing reads (bf16), or one element
 // of 32 consecutive channels (fp32).
-template <typename T, int DP, int R, int N>
+template <typename T, int DP, int R, typename P, int N>
 __device__ __forceinline__ void mma_cols(f32x16 (&acc)[N][DP / 32], const unsigned char* t, int r0,
-                                         const Probs<T> (&p)[N], int lane) {
+                                         const P (&p)[N], int lane) {
     using Tl = Tile<T, DP, R>;
     const int half = lane >> 5;
     if constexpr (kBf16Products<T>) {
@@ -244,7 +272,7 @@ __device__ __forceinline__ void mma_cols(f32x16 (&acc)[N][DP / 32], const unsign
                     f.p[q] = make_uint4(x.x, x.y, y.x, y.y);
                 }
 #pragma unroll
-                for (int n = 0; n < N; ++n) acc[n][b] = mma(f, p[n].v[s], acc[n][b]);
+                for (int n = 0; n < N; ++n) acc[n][b] = mma_probs(f, p[n], s, acc[n][b]);
             }
         }
     } else {

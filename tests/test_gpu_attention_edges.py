@@ -147,3 +147,21 @@ def test_the_largest_fp32_values(value, fits):
             assert bool(torch.isnan(got).all())
         out[0, :, 0, 5] = 0
         assert not out.any()
+
+
+@pytest.mark.parametrize("Nq,Nk,Hq,Hkv,D", [(1, 65, 8, 8, 64), (1, 4000, 8, 2, 64), (32, 77, 2, 2, 32), (4, 300, 8, 1, 128),
+                                            (3, 1000, 4, 4, 16), (1, 2, 8, 8, 8)])
+@pytest.mark.parametrize("living", [False, True], ids=["", "alive"])
+def test_bf16_weights_of_few_rows_in_two_parts(Nq, Nk, Hq, Hkv, D, living):
+    """At most 32 rows a key head: each weight is off by two roundings to bf16, one of the other's
+    rest (2^-16), so the output's own rounding is all that is left of that type."""
+    import slime_amd
+    B, dt = 3, torch.bfloat16
+    q, k, v = (_draw((B, n, h, D), dt, s) for n, h, s in ((Nq, Hq, 1), (Nk, Hkv, 2), (Nk, Hkv, 3)))
+    g = torch.Generator(device="cuda").manual_seed(4)
+    alive = torch.rand(B, Nk, generator=g, device="cuda") < 0.7 if living else None
+    r = ref.Reference(q, k, v, 1 / math.sqrt(D), ref.seen_mask(B, Nq, Nk, alive=alive))
+    out, _ = slime_amd.attend(q, k, v, alive=alive)
+    u = ref.u_of(dt)
+    tol = (2 * r.ds + (Nk + 32) * ref.U32 + u * u) * (r.p @ r.v.abs()) + u * r.out.abs() + 1e-30
+    ref.within(out, r.out.permute(0, 2, 1, 3), tol.permute(0, 2, 1, 3), "out")
