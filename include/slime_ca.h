@@ -389,8 +389,9 @@ typedef struct {
 
 /* Queries and keys in one pass: each head x normed, n = x w / sqrt(mean(x^2) + eps) with
  * the gains w (device fp32 [D]: wq, wk), and its pairs (u, v) turned by the angle
- * t = position * freq: (n_u cos t - n_v sin t, n_u sin t + n_v cos t). Angles are exact
- * to 2^-53 turns per position, also at positions near 2^31. B N D is below 2^35. */
+ * t = position * freq: (n_u cos t - n_v sin t, n_u sin t + n_v cos t). Angles are off by
+ * at most 2^-53 turns a position (a frequency's last bit) and 2^-32 turns (the phase's), at
+ * any position of 32 bits; their sine and cosine are fp32. B N D is below 2^35. */
 int slime_ca_qk_norm_rotate(const slime_ca_norm_config* config, const slime_ca_heads* q,
                             const slime_ca_heads* k, const float* wq, const float* wk,
                             const slime_ca_heads* q_out, const slime_ca_heads* k_out, void* stream);
@@ -426,16 +427,19 @@ typedef struct {
 } slime_ca_attend_config;
 
 /* out = softmax over the seen keys of (scale q . k) applied to v, and lse (device fp32
- * [B][Hq][Nq]), the log of the sum of exp(scale q . k): fp32 sums; bf16 probabilities are
- * rounded to bf16 before they meet v. In fp32 more than 32 rows of a key head (Nq Hq / Hkv)
- * run on the bf16 matrix cores, each value as the sum of three bf16 parts that hold its 24
- * bits: errors are as of fp32 products but for values below 2^-110, whose parts end at 2^-133
- * (bf16's smallest), and a value above 3.39e38 or infinite counts as NaN.
- * A query that sees no key gives 0 and -inf. One
- * query or few over many keys are split over the device, through the workspace (device,
+ * [B][Hq][Nq]), the log of the sum of exp(scale q . k): fp32 sums. A query that sees no key
+ * gives 0 and -inf.
+ *
+ * bf16 probabilities are rounded to bf16 before they meet v, in two parts (to 2^-16) where a
+ * key head has at most 32 rows (Nq Hq / Hkv). fp32 with more rows runs on the bf16 matrix
+ * cores, each value as the sum of three bf16 parts that hold its 24 bits: errors are as of
+ * fp32 products but for values below 2^-110, whose parts end at 2^-133 (bf16's smallest), and
+ * a value above 3.39e38 or infinite counts as NaN.
+ *
+ * One query or few over many keys are split over the device, through the workspace (device,
  * 16-byte aligned, slime_ca_attend_workspace bytes for the current device; may be 0). A batch
- * of more workgroups than one launch takes (2^24, of one head's queries each) goes in several;
- * one entry that exceeds a launch is SLIME_EINVAL. */
+ * of more workgroups than one launch takes (2^24, of one head's queries each) goes in
+ * several; one entry that exceeds a launch is SLIME_EINVAL. */
 int slime_ca_attend_workspace(const slime_ca_attend_config* config, int backward, size_t* bytes);
 int slime_ca_attend(const slime_ca_attend_config* config, const slime_ca_heads* q, const slime_ca_heads* k,
                     const slime_ca_heads* v, const slime_ca_heads* out, float* lse, void* workspace,
@@ -443,7 +447,9 @@ int slime_ca_attend(const slime_ca_attend_config* config, const slime_ca_heads* 
 
 /* The gradient of slime_ca_attend from its inputs, its out and lse and the gradient of
  * out; probabilities are computed again. grad_k and grad_v are summed over the query
- * heads that share a key head; keys that no query may see get 0. */
+ * heads that share a key head; keys that no query may see get 0. In bf16 the probabilities
+ * and the scores' gradients are rounded to bf16 before the products that sum them (fp32
+ * sums); in fp32 they are three parts, as above. */
 int slime_ca_attend_backward(const slime_ca_attend_config* config, const slime_ca_heads* grad_out,
                              const slime_ca_heads* q, const slime_ca_heads* k, const slime_ca_heads* v,
                              const slime_ca_heads* out, const float* lse, const slime_ca_heads* grad_q,

@@ -12,6 +12,9 @@ and ``attend_backward`` and ``qk_norm_rotate_backward`` give the gradients. All 
 the module ``_binding`` calls on torch's tensors; nothing synchronises, and every call may be
 captured into a graph.
 
+As ``Pseudopod``'s, the calls are outside autograd: outputs require no grad, and the gradients are
+calls of their own.
+
 Tensors are CUDA tensors [B, N, heads, D] (N cells or states), float32 or bfloat16, with any
 strides but 1 along D: planes [B, G, G, C] viewed per head, parts of one packed product, or heads
 first. D is 8, 16, 32, 64 or 128; Hq query heads share Hkv key heads, Hq % Hkv == 0. ``stream``

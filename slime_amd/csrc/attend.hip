@@ -8,8 +8,8 @@
 // (attend.hpp): every lane has one row's statistics, and P stays in its registers.
 //
 // What bounds it. Many rows: matrix cores and arithmetic share the card's power. 16,384^2 x 8 x 64
-// in bf16 takes 578 us (951 TFLOP/s; a library product of 8192^3 reaches 1215); the same products
-// and tiles without exponentials, LDS reads and loads take 440. Two sets of rows a wave halve the
+// in bf16 takes 578 to 593 us from card to card (927 to 951 TFLOP/s; a library product of 8192^3
+// reaches 1215); the same products and tiles without exponentials, LDS reads and loads take 440. Two sets of rows a wave halve the
 // LDS reads (one set 695 us, two 587 of one build). Three blocks of keys in flight (scores,
 // weights and product at once) spilled: 656. Deferring the maximum, or two tiles under way
 // instead of one, changed nothing. Few rows: the keys' bytes; 16 histories of 8,192 to 16,384,
@@ -474,8 +474,9 @@ AttendPlan attend_plan(int dtype, const AttendArgs& a, int n_cu) {
     if (two_sets(dtype == 1 ? 2 : 4, a.D) && heads * ((rows + 255) / 256) >= 2LL * n_cu) p.rows = 256;
     // The number of splits, each of two tiles of keys at least, that takes the least time, in products of
     // a tile by 128 rows: a workgroup starts and ends in the time of two. Walks of one length go in
-    // rounds of the workgroups that are resident at once (two on a CU; one of fp32 heads of 128, which fill
-    // the registers), of which half of one takes 0.8 of its time, or 0.6 where few rows wait for memory;
+    // rounds of two workgroups a CU (one of fp32 heads of 128, which fill the registers), of which half of
+    // one takes 0.8 of its time, or 0.6 where few rows wait for memory; few rows of wide heads (bf16 of
+    // 128, fp32 of 64), of which LDS holds one workgroup a CU, have the same fit: a round is two in turn there;
     // walks of many lengths, longest first, end in a quarter of the longest. The parts take 0.15 a
     // thousand rows (fp32 products three times as long beside them) and their join two. Against one
     // workgroup on a CU, or two in fp32 above 32 channels and for few rows, us: 4096 causal x 8 x 64 in

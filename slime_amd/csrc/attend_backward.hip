@@ -10,9 +10,13 @@
 // of workgroups run in one launch, so that a small call's fill the device together and a large
 // call's last ones leave no gap.
 //
-// What bounds it: 4 x 4096^2 x 8 x 64 in bf16 takes 479 us, 1050 TFLOP/s of the products that it
-// makes (a library product of 8192^3 reaches 1215), 717 of the five that it cannot do without.
-// 6144 causal, 8 over 2 heads of 128, takes 368: 3 + 5 products, and 20 for the parts' sums.
+// What bounds it: 4 x 4096^2 x 8 x 64 in bf16 takes 480 to 507 us from card to card, 1015 to 1070
+// TFLOP/s of the products that it makes (a library product of 8192^3 reaches 1215), 680 to 715 of
+// the five that it cannot do without. 6144 causal, 8 over 2 heads of 128, takes 364 to 374: 3 + 5
+// products, and 20 for the parts' sums.
+//
+// P and dS are rounded to bf16 before the products that sum them, the type of those products' other
+// operands: gradients are off by 1.4 of their own rounding. In fp32 they are three parts.
 #include "attend.hpp"
 
 namespace slime {
@@ -216,7 +220,10 @@ __device__ __forceinline__ void grad_q(const AttendArgs& a, int row_tiles, int h
 // A workgroup takes both gradients of its keys (four products a tile), or where those exceed a
 // wave's 256 registers one the keys' gradient (three products) and its neighbour the values'
 // (two): one product more (heads of 128: 435 us in one role, which moves its accumulators in and
-// out, 398 in two; heads of 64: 507 in one, 609 in two with 64 keys a wave, 770 with 32).
+// out, 398 in two; heads of 64: 507 in one, 609 in two with 64 keys a wave, 770 with 32). Not all
+// fit even so: of heads of 128 in bf16 a lane has 8 registers in scratch memory, 22 with living
+// cells, of heads of 64 with living cells 6; in fp32 2 for heads of 64 and 16 to 33 of 512 for 128.
+// KB is 1 in every call.
 enum Part { kBoth, kValues, kKeysOnly };
 
 template <typename T, int DP, int KB>
@@ -423,7 +430,7 @@ __device__ __forceinline__ void grad_kv(const AttendArgs& a, int head, int item,
 }
 
 // How the workgroups share the keys' and the values' gradients: by keys alone, but by roles too
-// where both gradients' accumulators and the keys' and values' operands exceed 256 registers.
+// where both gradients' accumulators and the keys' and values' operands exceed 256 registers by far.
 template <typename T, int DP>
 constexpr int kRoles = DP * Elem<T>::kPlanes >= 128 ? 2 : 1;
 

@@ -23,8 +23,8 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 2;
 
 // Sine and cosine of pos * freq (radians). The phase is a 64-bit fraction of a turn, and so
-// exact modulo whole turns at any position: freq / 2 pi keeps its 53 bits. The quarter turn
-// nearest to it leaves |x| <= pi / 4 for the Taylor series, whose next terms are 2e-9 and
+// exact modulo whole turns at any position: freq / 2 pi keeps its 53 bits, the phase 32.
+// The quarter turn nearest to it leaves |x| <= pi / 4 for the Taylor series, whose next terms are 2e-9 and
 // 2e-10.
 __device__ __forceinline__ void turn_of(int pos, double freq, float& s, float& c) {
     double f = freq * 0.15915494309189533577;  // 1 / 2 pi
